@@ -24,21 +24,13 @@ DTYPES = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32}
 BALANCE, ZLOSS = 1e-2, 1e-3
 
 
-_modules = None
-
-
 def _package():
-    """The framework's modules, looked up once: a user's program imports them at its start, not in every step."""
-    global _modules
-    if _modules is not None:
-        return _modules
     here = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "grouped-gemms_b200")
     if here not in sys.path:
         sys.path.insert(0, here)
     import kernels
     import mxgg.moe
-    _modules = (mxgg.moe, kernels)
-    return _modules
+    return mxgg.moe, kernels
 
 
 # ------------------------------------------------------------------- cases
