@@ -197,7 +197,9 @@ __global__ void __launch_bounds__(KC <= 4 ? kRowsMaxThreads : 256) lora_rows_ker
       }
     }
     const int r = i * 4 / p.Rp, c = i * 4 % p.Rp;
-    *reinterpret_cast<float4*>(&sh_v[r][c]) = make_float4(scale * s.x, scale * s.y, scale * s.z, scale * s.w);
+    // ranks past R stay 0: their sums of x times 0 are NaN beside an infinite x
+    if (c < p.R)
+      *reinterpret_cast<float4*>(&sh_v[r][c]) = make_float4(scale * s.x, scale * s.y, scale * s.z, scale * s.w);
   }
   ptx::cluster_arrive();                                  // waited for at the end: no CTA leaves while it is read
   __syncthreads();

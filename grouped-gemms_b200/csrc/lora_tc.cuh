@@ -99,7 +99,9 @@ __device__ __forceinline__ uint32_t smem_align1024(const void* p) { return (ptx:
 // ------------------------------------------------------------------ shrink
 // A cluster of `ksplit` CTAs owns 128 rows; each CTA multiplies its share of
 // the contraction and the cluster adds the partial tiles through distributed
-// shared memory, in rank order, before one rounding to v's halves.
+// shared memory, in rank order, before one rounding to v's halves.  The ranks
+// past R are set to 0 there: their sums of x times 0 are NaN beside an infinite x,
+// and would make a NaN of the whole row in the second product.
 // Bound: HBM, x once.  16384 x 5120, rank 16: 36 us, 4.7 TB/s (a plain read of
 // as much, 28 us; about 8 us are the launch's start and the join); 16384 x 8192:
 // 57 us.  Three to five stages, one or two CTAs to an SM measured the same.
@@ -252,7 +254,7 @@ __global__ void __launch_bounds__(128) lora_shrink_kernel(const __grid_constant_
         for (int h = 0; h < 2; ++h) {
           float f[8];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) f[i] = scale * __uint_as_float(r[h * 8 + i]);
+          for (int i = 0; i < 8; ++i) f[i] = c + h * 8 < p.R ? scale * __uint_as_float(r[h * 8 + i]) : 0.0f;
           uint4 hi, lo;
           split_halves(f, hi, lo);
           *reinterpret_cast<uint4*>(row + c + h * 8) = hi;
@@ -297,7 +299,7 @@ __global__ void __launch_bounds__(128) lora_shrink_kernel(const __grid_constant_
       const int m = row0 + rr;
       if (m < end) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) f[j] *= scale;
+        for (int j = 0; j < 8; ++j) f[j] = c < p.R ? f[j] * scale : 0.0f;
         uint4 hi, lo;
         split_halves(f, hi, lo);
         __nv_bfloat16* row = p.v + (long long)m * vld;
