@@ -40,8 +40,6 @@ namespace {
 // device-side error word raised by bounded waits
 __device__ uint32_t g_status_word;
 
-constexpr int kMaxDevices = 64;
-
 std::mutex g_mu;
 DeviceState g_dev[kMaxDevices];
 
@@ -109,6 +107,7 @@ int get_device_state(DeviceState** out) {
       MXGG_CUDA_TRY(cudaGetDriverEntryPoint("cuStreamWriteValue32", &fn, cudaEnableDefault, &q));
       if (q == cudaDriverEntryPointSuccess && fn) g_write_value = reinterpret_cast<WriteValueFn>(fn);
     }
+    st.device = dev;
     st.init = true;
   }
   *out = &st;

@@ -62,6 +62,14 @@ int out_es(int t) { return t == MXGG_DTYPE_F32 ? 4 : 2; }
 constexpr CUtensorMapDataType kBf16Map = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
 constexpr CUtensorMapSwizzle kSwz = CU_TENSOR_MAP_SWIZZLE_128B;
 
+// Shared memory of a CTA's ring and tables, at most: two CTAs to an SM, and one.
+// A stage of the shrink is 32 KB at most, so it has three; the expand's tiles of
+// v count too.
+constexpr int kShrinkSmem = 96 * 1024;
+static_assert(kShrinkSmem / (kShrinkXBytes + kMaxLoraRank * 128) >= 3, "stages of the shrink");
+constexpr int kExpandPairSmem = 98 * 1024, kExpandSmem = 212 * 1024;
+constexpr int kWgradSmem = 108 * 1024;
+
 int run_shrink(DeviceState* st, const LoraSegs& g, const void* x, int64_t ld, const void* w, int r_contig,
                const float* scaling, int64_t C, int64_t R, void* v, cudaStream_t stream) {
   ShrinkParams p{};
@@ -82,7 +90,7 @@ int run_shrink(DeviceState* st, const LoraSegs& g, const void* x, int64_t ld, co
   while (p.ksplit < 8 && tiles * p.ksplit < st->num_sms && kiters / (2 * p.ksplit) >= 4) p.ksplit *= 2;
   // two CTAs share an SM
   const int stage = kShrinkXBytes + p.w_bytes;
-  p.stages = std::max(3, std::min(kShrinkMaxStages, 96 * 1024 / stage));
+  p.stages = std::min(kShrinkMaxStages, kShrinkSmem / stage);
   const size_t smem = (size_t)p.stages * stage + 1024;
   CUtensorMap mx, mx32, mw;
   if (int rc = make_tmap_2d(&mx, x, kBf16Map, 2, (uint64_t)g.M, (uint64_t)C, (uint64_t)ld, kLoraBK, kLoraBM, kSwz))
@@ -94,7 +102,7 @@ int run_shrink(DeviceState* st, const LoraSegs& g, const void* x, int64_t ld, co
                         : make_tmap_3d(&mw, w, kBf16Map, 2, (uint64_t)g.L, (uint64_t)R, (uint64_t)C, (uint64_t)C,
                                        (uint64_t)(C * R), kLoraBK, (uint32_t)p.Rp, 1, kSwz))
     return rc;
-  MXGG_CUDA_TRY(cudaFuncSetAttribute(lora_shrink_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  if (int rc = allow_smem<lora_shrink_kernel>(*st, kShrinkSmem + 1024)) return rc;
   MXGG_CUDA_TRY(launch(lora_shrink_kernel, dim3((unsigned)(tiles * p.ksplit)), dim3(128), smem, p.ksplit, false, stream,
                        mx, mx32, mw, p));
   return MXGG_OK;
@@ -116,9 +124,10 @@ int make_v_map(CUtensorMap* m, const void* v, int M, int Rp, int rows) {
                       (uint32_t)rows, kSwz);
 }
 
-int run_expand(DeviceState* st, const LoraSegs& g, const void* v, const void* w, int r_contig, const void* base,
-               int64_t base_ld, void* out, int64_t out_ld, int out_dtype, int64_t C, int64_t R, bool more,
-               cudaStream_t stream) {
+template <typename O>
+int expand_as(DeviceState* st, const LoraSegs& g, const void* v, const void* w, int r_contig, const void* base,
+              int64_t base_ld, void* out, int64_t out_ld, int out_dtype, int64_t C, int64_t R, bool more,
+              cudaStream_t stream) {
   ExpandParams p{};
   p.more = more;
   p.g = g;
@@ -142,8 +151,8 @@ int run_expand(DeviceState* st, const LoraSegs& g, const void* v, const void* w,
   p.nsplit = (int)std::max<long long>(1, std::min<long long>((nt + 1) / 2, 2LL * st->num_sms / tiles));
   const int vb = p.v_pieces * kLoraBM * 128, stage = p.base_bytes + p.w_bytes;
   // two CTAs share an SM where that leaves each three stages
-  const int pair = (98 * 1024 - vb) / stage;
-  p.stages = std::min(kExpandMaxStages, pair >= 3 ? pair : (212 * 1024 - vb) / stage);
+  const int pair = (kExpandPairSmem - vb) / stage;
+  p.stages = std::min(kExpandMaxStages, pair >= 3 ? pair : (kExpandSmem - vb) / stage);
   const size_t smem = (size_t)vb + (size_t)p.stages * stage + 1024;
   CUtensorMap mv, mw, mb, mb32, mo;
   if (int rc2 = make_v_map(&mv, v, g.M, p.Rp, kLoraBM)) return rc2;
@@ -168,13 +177,19 @@ int run_expand(DeviceState* st, const LoraSegs& g, const void* v, const void* w,
                                  (uint32_t)(128 / es), 32, kSwz))
         return rc2;
   }
-  auto k = out_dtype == MXGG_DTYPE_BF16  ? lora_expand_kernel<__nv_bfloat16>
-           : out_dtype == MXGG_DTYPE_F16 ? lora_expand_kernel<__half>
-                                         : lora_expand_kernel<float>;
-  MXGG_CUDA_TRY(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-  MXGG_CUDA_TRY(launch(k, dim3((unsigned)(tiles * p.nsplit)), dim3(kExpandThreads), smem, 1, true, stream, mv, mw, mb,
-                       mb32, mo, p));
+  if (int rc2 = allow_smem<lora_expand_kernel<O>>(*st, kExpandSmem + 1024)) return rc2;
+  MXGG_CUDA_TRY(launch(lora_expand_kernel<O>, dim3((unsigned)(tiles * p.nsplit)), dim3(kExpandThreads), smem, 1, true,
+                       stream, mv, mw, mb, mb32, mo, p));
   return MXGG_OK;
+}
+
+int run_expand(DeviceState* st, const LoraSegs& g, const void* v, const void* w, int r_contig, const void* base,
+               int64_t base_ld, void* out, int64_t out_ld, int out_dtype, int64_t C, int64_t R, bool more,
+               cudaStream_t stream) {
+  auto f = out_dtype == MXGG_DTYPE_BF16  ? expand_as<__nv_bfloat16>
+           : out_dtype == MXGG_DTYPE_F16 ? expand_as<__half>
+                                         : expand_as<float>;
+  return f(st, g, v, w, r_contig, base, base_ld, out, out_ld, out_dtype, C, R, more, stream);
 }
 
 // Launch shape of the weight gradients: no more CTAs than there are stages.
@@ -210,7 +225,7 @@ int run_wgrad(DeviceState* st, const LoraSegs& g, const WgradArgs* jobs, int n, 
   p.wait_ns = wait_limit_ns();
   const int stage = kWgradZBytes + lora_v_pieces(p.Rp) * kWgradBT * 128;
   const int tables = wgrad_table_bytes(g.S);
-  p.stages = std::min(kWgradMaxStages, (108 * 1024 - tables) / stage);   // two CTAs to an SM
+  p.stages = std::min(kWgradMaxStages, (kWgradSmem - tables) / stage);   // two CTAs to an SM
   const size_t smem = (size_t)p.stages * stage + tables + 1024;
   CUtensorMap mv[2], mz[2];
   long long sum_blocks = 0;
@@ -235,7 +250,7 @@ int run_wgrad(DeviceState* st, const LoraSegs& g, const WgradArgs* jobs, int n, 
     mv[1] = mv[0];
     mz[1] = mz[0];
   }
-  MXGG_CUDA_TRY(cudaFuncSetAttribute(lora_wgrad_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  if (int rc = allow_smem<lora_wgrad_kernel>(*st, kWgradSmem + 1024)) return rc;
   MXGG_CUDA_TRY(launch(lora_wgrad_kernel, dim3((unsigned)ctas), dim3(kWgradThreads), smem, 1, pdl, stream, mv[0],
                        mz[0], mv[1], mz[1], p));
   auto k = out_dtype == MXGG_DTYPE_BF16  ? lora_wgrad_sum_kernel<__nv_bfloat16>
@@ -261,18 +276,18 @@ bool rows_form(const int32_t* offs, int64_t S, int64_t M, int64_t R) {
   return M <= 256 && (M <= 32 * S || M * lora_rp((int)R) <= 8192);
 }
 
-template <typename O>
-int rows_as(RowsParams p, cudaStream_t stream) {
-  auto k = p.Rp <= 16   ? lora_rows_kernel<O, 1>
-           : p.Rp <= 32 ? lora_rows_kernel<O, 2>
-           : p.Rp <= 64 ? lora_rows_kernel<O, 4>
-                        : lora_rows_kernel<O, 8>;
-  const int threads = p.Rp <= 64 ? p.threads : 256;
-  const size_t smem = (size_t)(threads / 32) * kRowsGroup * rows_red_ld(p.Rp) * 4;
-  MXGG_CUDA_TRY(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+constexpr int rows_threads(int KC, int wanted) { return KC <= 4 ? wanted : 256; }
+constexpr int rows_smem(int threads, int Rp) { return threads / 32 * kRowsGroup * rows_red_ld(Rp) * 4; }
+
+template <typename O, int KC>
+int rows_launch(const DeviceState& st, RowsParams p, cudaStream_t stream) {
+  auto k = lora_rows_kernel<O, KC>;
+  const int threads = rows_threads(KC, p.threads);
+  const size_t smem = rows_smem(threads, p.Rp);
+  if (int rc = allow_smem<lora_rows_kernel<O, KC>>(st, rows_smem(rows_threads(KC, kRowsMaxThreads), 16 * KC), true))
+    return rc;
   if (p.cluster > 8) {
     // a device (or a slice of one) without 16 free SMs in a GPC takes clusters of 8
-    MXGG_CUDA_TRY(cudaFuncSetAttribute(k, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     const cudaError_t e = launch(k, dim3((unsigned)p.g.M * (unsigned)p.cluster), dim3(threads), smem, p.cluster, false,
                                  stream, p);
     if (e == cudaSuccess) return MXGG_OK;
@@ -282,6 +297,14 @@ int rows_as(RowsParams p, cudaStream_t stream) {
   }
   MXGG_CUDA_TRY(launch(k, dim3((unsigned)p.g.M * (unsigned)p.cluster), dim3(threads), smem, p.cluster, false, stream, p));
   return MXGG_OK;
+}
+
+template <typename O>
+int rows_as(const DeviceState& st, const RowsParams& p, cudaStream_t stream) {
+  return p.Rp <= 16   ? rows_launch<O, 1>(st, p, stream)
+         : p.Rp <= 32 ? rows_launch<O, 2>(st, p, stream)
+         : p.Rp <= 64 ? rows_launch<O, 4>(st, p, stream)
+                      : rows_launch<O, 8>(st, p, stream);
 }
 
 }  // namespace
@@ -340,9 +363,9 @@ int mxgg_lora_mm(const void* x, int64_t x_ld, const void* a, const void* b, cons
     p.cluster = M <= kRowsFew ? 16 : 8;
     p.threads = M <= kRowsFew ? 512 : 256;
     switch (out_dtype) {
-      case MXGG_DTYPE_BF16: return rows_as<__nv_bfloat16>(p, stream);
-      case MXGG_DTYPE_F16: return rows_as<__half>(p, stream);
-      default: return rows_as<float>(p, stream);
+      case MXGG_DTYPE_BF16: return rows_as<__nv_bfloat16>(*st, p, stream);
+      case MXGG_DTYPE_F16: return rows_as<__half>(*st, p, stream);
+      default: return rows_as<float>(*st, p, stream);
     }
   }
   if (int rc = run_shrink(st, g, x, x_ld, a, 0, scaling, K, R, v, stream)) return rc;

@@ -275,8 +275,7 @@ int mxgg_dispatch_plan(const int32_t* chosen, int64_t tokens, int32_t k, int64_t
   p.pair_pos = pair_pos;
   const int blocks = std::max(1, (p.pairs + p.per - 1) / p.per);
   const int smem = (kPlanWarps + 3) * p.E * 4;
-  if (smem > 48 * 1024)
-    MXGG_CUDA_TRY(cudaFuncSetAttribute(plan_place_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  if (int rc = allow_smem<plan_place_kernel>(*st, (kPlanWarps + 3) * kMaxRouteExperts * 4)) return rc;
   if (blocks == 1) {
     plan_place_kernel<<<1, kPlanThreads, smem, stream>>>(p);
     MXGG_CUDA_TRY(cudaGetLastError());

@@ -5,6 +5,7 @@
 #include <cuda.h>
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cstdint>
 
 #include "../../include/mxgg.h"
@@ -22,6 +23,7 @@ int fail(int code, const char* fmt, ...);
 
 struct DeviceState {
   bool init = false;
+  int device = 0;
   int num_sms = 0;
   uint32_t* status = nullptr;   // device address of the status word bounded waits raise
 };
@@ -39,6 +41,22 @@ int make_tmap_3d(CUtensorMap* map, const void* base, CUtensorMapDataType dt, int
                  uint32_t box_rows, uint32_t box_mats, CUtensorMapSwizzle swz);
 
 inline bool aligned(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
+
+// Allows `kernel` `bytes` of dynamic shared memory (and clusters of more than 8
+// CTAs), on the first call for a device.  `bytes` is the most that any launch of
+// it takes, never one call's own size: the limit belongs to the function, and a
+// call that lowered it between another thread's setting and launch would make
+// that launch fail.  Two first calls at once both set the same.
+constexpr int kMaxDevices = 64;
+template <auto kernel>
+int allow_smem(const DeviceState& st, int bytes, bool large_cluster = false) {
+  static std::atomic<bool> done[kMaxDevices] = {};
+  if (done[st.device].load(std::memory_order_acquire)) return MXGG_OK;
+  MXGG_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  if (large_cluster) MXGG_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+  done[st.device].store(true, std::memory_order_release);
+  return MXGG_OK;
+}
 
 // Launch with a cluster along x and/or programmatic stream serialisation: the
 // kernel may then start while the stream's previous kernel drains, and must
