@@ -3,7 +3,10 @@
 // thread issuing the loads and one the products.
 //
 // Every wait is bounded: one that runs out sets kErrLoraWait in the device
-// status word and the kernel drains its copies, frees its TMEM and returns.
+// status word and ends the roles' loops.  Behind the barrier that all of them
+// reach, the copies still in flight are waited for (whichever role's wait ran
+// out, also after the last load was issued), then the kernel frees its TMEM and
+// returns: shared memory that a copy may still write never goes to another CTA.
 #pragma once
 
 #include "lora.cuh"
@@ -96,6 +99,14 @@ __device__ __forceinline__ void split_halves(const float (&f)[8], uint4& hi, uin
 
 __device__ __forceinline__ uint32_t smem_align1024(const void* p) { return (ptx::smem_u32(p) + 1023u) & ~1023u; }
 
+// Waits (bounded) for a ring's loads that may be in flight, the last ones issued:
+// load j went to stage j % stages in that stage's round j / stages.
+__device__ __forceinline__ void lora_drain(uint64_t* full, int issued, int stages, unsigned long long wait_ns) {
+  volatile int never = 0;
+  for (int j = max(0, issued - stages); j < issued; ++j)
+    ptx::mbar_wait(ptx::smem_u32(full + j % stages), (j / stages) & 1, &never, wait_ns);
+}
+
 // ------------------------------------------------------------------ shrink
 // A cluster of `ksplit` CTAs owns 128 rows; each CTA multiplies its share of
 // the contraction and the cluster adds the partial tiles through distributed
@@ -127,7 +138,7 @@ __global__ void __launch_bounds__(128) lora_shrink_kernel(const __grid_constant_
   __shared__ int sh_start[kMaxLoraSegments + 1], sh_tiles[kMaxLoraSegments + 1], sh_ad[kMaxLoraSegments];
   __shared__ alignas(8) uint64_t sh_full[kShrinkMaxStages], sh_empty[kShrinkMaxStages], sh_done;
   __shared__ uint32_t sh_tmem;
-  __shared__ int sh_abort;
+  __shared__ int sh_abort, sh_issued;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int kq = blockIdx.x % p.ksplit, tile = blockIdx.x / p.ksplit;
   const uint32_t ring = smem_align1024(smem_raw);
@@ -178,7 +189,6 @@ __global__ void __launch_bounds__(128) lora_shrink_kernel(const __grid_constant_
 
   if (warp == 0) {
     if (lane == 0) {
-      volatile int never = 0;
       int issued = 0;
       for (int i = i0; i < i1; ++i, ++issued) {
         const int st = issued % p.stages, round = issued / p.stages;
@@ -203,9 +213,7 @@ __global__ void __launch_bounds__(128) lora_shrink_kernel(const __grid_constant_
           ptx::tma_load_3d(dst + kShrinkXBytes, &map_w, full, i * kLoraBK, 0, l);
         }
       }
-      if (*abort)     // copies in flight must land before this CTA's shared memory goes
-        for (int j = max(0, issued - p.stages); j < issued; ++j)
-          ptx::mbar_wait(ptx::smem_u32(&sh_full[j % p.stages]), (j / p.stages) & 1, &never, p.wait_ns);
+      sh_issued = issued;
     }
     __syncwarp();
   } else if (warp == 1) {
@@ -311,6 +319,10 @@ __global__ void __launch_bounds__(128) lora_shrink_kernel(const __grid_constant_
   }
   ptx::tc_fence_before();
   __syncthreads();
+  if (sh_abort) {
+    if (tid == 0) lora_drain(sh_full, sh_issued, p.stages, p.wait_ns);
+    __syncthreads();
+  }
   if (warp == 2) ptx::tmem_dealloc(tmem, ncols);
 }
 
@@ -375,7 +387,7 @@ lora_expand_kernel(const __grid_constant__ CUtensorMap map_v, const __grid_const
   __shared__ alignas(8) uint64_t sh_full[kExpandMaxStages], sh_empty[kExpandMaxStages];
   __shared__ alignas(8) uint64_t sh_acc_full[2], sh_acc_empty[2], sh_v;
   __shared__ uint32_t sh_tmem;
-  __shared__ int sh_abort;
+  __shared__ int sh_abort, sh_issued;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int part = blockIdx.x % p.nsplit, tile = blockIdx.x / p.nsplit;
   if (warp == 0) lora_build_table(p.g, kLoraBM, sh_start, sh_tiles, sh_ad);
@@ -474,12 +486,7 @@ lora_expand_kernel(const __grid_constant__ CUtensorMap map_v, const __grid_const
                              p.v_pieces == 1 ? 0 : j / rc, row0);
         }
       }
-      if (*abort) {
-        volatile int never = 0;
-        ptx::mbar_wait(ptx::smem_u32(&sh_v), 0, &never, p.wait_ns);
-        for (int j = max(0, issued - p.stages); j < issued; ++j)
-          ptx::mbar_wait(ptx::smem_u32(&sh_full[j % p.stages]), (j / p.stages) & 1, &never, p.wait_ns);
-      }
+      sh_issued = issued;
     }
     __syncwarp();
   } else if (warp == 1) {
@@ -605,13 +612,17 @@ lora_expand_kernel(const __grid_constant__ CUtensorMap map_v, const __grid_const
   ptx::griddep_wait();
   ptx::tc_fence_before();
   __syncthreads();
-  if (sh_abort && tid == 32) {
-    // products in flight must end before their accumulators go
-    volatile int never = 0;
-    ptx::tc_commit(ptx::smem_u32(&sh_v));
-    ptx::mbar_wait(ptx::smem_u32(&sh_v), 1, &never, p.wait_ns);
+  if (sh_abort) {
+    if (tid == 32) {
+      // v's load, the ring's, and (before their accumulators go) the products in flight
+      volatile int never = 0;
+      ptx::mbar_wait(ptx::smem_u32(&sh_v), 0, &never, p.wait_ns);
+      lora_drain(sh_full, sh_issued, p.stages, p.wait_ns);
+      ptx::tc_commit(ptx::smem_u32(&sh_v));
+      ptx::mbar_wait(ptx::smem_u32(&sh_v), 1, &never, p.wait_ns);
+    }
+    __syncthreads();
   }
-  __syncthreads();
   if (warp == 2) ptx::tmem_dealloc(tmem, 2 * kExpandBN);
 }
 
@@ -675,7 +686,7 @@ lora_wgrad_kernel(const __grid_constant__ CUtensorMap map_v0, const __grid_const
   __shared__ alignas(8) uint64_t sh_full[kWgradMaxStages], sh_empty[kWgradMaxStages];
   __shared__ alignas(8) uint64_t sh_acc_full[2], sh_acc_empty[2], sh_done;
   __shared__ uint32_t sh_tmem;
-  __shared__ int sh_abort;
+  __shared__ int sh_abort, sh_issued;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int rc = (p.Rp + 63) / 64;
   const uint32_t ring = smem_align1024(smem_raw + wgrad_table_bytes(p.g.S));
@@ -802,11 +813,7 @@ lora_wgrad_kernel(const __grid_constant__ CUtensorMap map_v0, const __grid_const
           t += w.n;
         }
       }
-      if (*abort) {
-        volatile int never = 0;
-        for (int j = max(0, issued - p.stages); j < issued; ++j)
-          ptx::mbar_wait(ptx::smem_u32(&sh_full[j % p.stages]), (j / p.stages) & 1, &never, p.wait_ns);
-      }
+      sh_issued = issued;
     }
     __syncwarp();
   } else if (warp == 1) {
@@ -927,10 +934,17 @@ lora_wgrad_kernel(const __grid_constant__ CUtensorMap map_v0, const __grid_const
   ptx::griddep_wait();
   {
     volatile int never = 0;
-    if (!ptx::mbar_wait(ptx::smem_u32(&sh_done), 0, &never, kLoraWaitSpan * p.wait_ns)) atomicOr(p.status, kErrLoraWait);
+    if (!ptx::mbar_wait(ptx::smem_u32(&sh_done), 0, &never, kLoraWaitSpan * p.wait_ns)) {
+      atomicOr(p.status, kErrLoraWait);
+      sh_abort = 1;
+    }
   }
   ptx::tc_fence_before();
   __syncthreads();
+  if (sh_abort) {
+    if (tid == 0) lora_drain(sh_full, sh_issued, p.stages, p.wait_ns);
+    __syncthreads();
+  }
   if (warp == 2) ptx::tmem_dealloc(tmem, ncols);
 }
 
