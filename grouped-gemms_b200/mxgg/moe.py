@@ -23,6 +23,7 @@ plain functions: a gradient is a call, not an autograd node.
 
 import ctypes
 from dataclasses import dataclass
+from functools import lru_cache
 from typing import NamedTuple, Optional, Tuple, Union
 
 import torch
@@ -101,7 +102,7 @@ class Routing(NamedTuple):
     counts: Tensor         # (E,) int32 choices of each expert
     balance_loss: Tensor   # () fp32: E * sum_e f_e P_e
     z_loss: Tensor         # () fp32: mean of logsumexp^2
-    buffer: Tensor         # int32: the allocation the fields are views of, with what the backward pass reads
+    buffer: Tensor         # int32: the allocation the fields are views of; the backward pass reads it, so leave it as it is
     renormalise: bool
 
     @property
@@ -121,6 +122,13 @@ def _routing_parts(T: int, k: int, E: int) -> tuple:
     (balance, z, tokens), scratch."""
     tk, st, e = (T * k + 3) & ~3, (2 * T + 3) & ~3, (E + 3) & ~3
     return 0, tk, 2 * tk, 2 * tk + st, 2 * tk + st + e, 2 * tk + st + e + 4
+
+
+@lru_cache(maxsize=256)
+def _routing_sizes(T: int, k: int, E: int) -> Tuple[tuple, int]:
+    """A Routing buffer's parts and the bytes of its scratch (negative: no such size); they follow from the
+    sizes alone, and asking for them anew takes 1.5 us of a call's host time."""
+    return _routing_parts(T, k, E), _lib.load().mxgg_route_workspace_size(T, E)
 
 
 def route_topk(logits: Tensor, k: int, token_mask: Optional[Tensor] = None, renormalise: bool = True) -> Routing:
@@ -149,8 +157,7 @@ def route_topk(logits: Tensor, k: int, token_mask: Optional[Tensor] = None, reno
     lib = _lib.load()
     # One allocation for every output and the scratch: an allocation costs 2.4 us of host time, a view of it
     # 1 us, the kernel of a decode step 6 us.
-    ws_bytes = lib.mxgg_route_workspace_size(T, E)
-    at = _routing_parts(T, k, E)
+    at, ws_bytes = _routing_sizes(T, k, E)
     with _on(dev):
         ints = torch.empty(at[5] + max(ws_bytes, 0) // 4, dtype=torch.int32, device=dev)
         floats = ints.view(torch.float32)
@@ -173,18 +180,36 @@ def _rows(t: Tensor) -> Tuple[Tensor, int]:
     return t, (t.stride(0) if T > 1 else E)
 
 
+def _routing_record(what: str, routing: Routing) -> Tuple[int, int, int, tuple]:
+    """(T, k, E, parts) of a Routing whose buffer is what route_topk wrote, or an error."""
+    buf, choices, counts = routing.buffer, routing.experts.shape, routing.counts.shape
+    if len(choices) != 2 or len(counts) != 1:
+        raise ValueError(f"{what}: routing holds experts {tuple(choices)} and counts {tuple(counts)}, not (tokens, k) "
+                         "and (experts,)")
+    (T, k), E = choices, counts[0]
+    at, ws_bytes = _routing_sizes(T, k, E)
+    # the whole size: a record of more tokens than the fields have lies otherwise
+    if buf.dtype != torch.int32 or buf.shape != (at[5] + max(ws_bytes, 0) // 4,) or not buf.is_contiguous():
+        raise ValueError(f"{what}: routing.buffer must be the int32 tensor of route_topk for ({T}, {k}) choices of {E} "
+                         f"experts, got {buf.dtype} {tuple(buf.shape)}")
+    if not buf.is_inference() and buf._version != 0:
+        raise ValueError(f"{what}: a tensor of routing was changed in place; the gradient is that of route_topk's own "
+                         "weights, counts and choices, so change a copy")
+    return T, k, E, at
+
+
 def route_topk_backward(logits: Tensor, routing: Routing, grad_weights: Optional[Tensor] = None,
                         grad_balance_loss: Union[Tensor, float, None] = None,
                         grad_z_loss: Union[Tensor, float, None] = None) -> Tensor:
     """Gradient to the logits of `route_topk(logits, ...) -> routing` ((T, E), the logits' dtype), for the
     gradients of its weights ((T, k) fp32) and of its two losses (a float, or a one-element fp32 tensor on
     the GPU).  None: no gradient there.  Choices and counts are constants.  Zero rows for tokens that do
-    not count."""
+    not count.  All it needs of `routing` it reads from `routing.buffer`: a Routing with other tensors in the
+    fields' places gives the same gradient, and one whose tensors were changed in place is refused."""
     what = "mxgg.moe.route_topk_backward"
+    T, k, E, at = _routing_record(what, routing)
     scalars = [g if isinstance(g, Tensor) else None for g in (grad_balance_loss, grad_z_loss)]
-    dev = _one_device(what, logits, routing.experts, grad_weights, *scalars)
-    T, k = routing.experts.shape
-    E = routing.counts.shape[0]
+    dev = _one_device(what, logits, routing.buffer, grad_weights, *scalars)
     if logits.dtype not in _IN_DTYPES:
         raise TypeError(f"{what}: unsupported logits dtype {logits.dtype}")
     if logits.shape != (T, E):
@@ -200,13 +225,12 @@ def route_topk_backward(logits: Tensor, routing: Routing, grad_weights: Optional
                 raise ValueError(f"{what}: a loss gradient is a float or a one-element tensor")
             scalars[i] = g.to(torch.float32)
     coef = [1.0 if isinstance(g, Tensor) else float(g or 0.0) for g in (grad_balance_loss, grad_z_loss)]
-    at, p = _routing_parts(T, k, E), routing.buffer.data_ptr()
+    p = routing.buffer.data_ptr()
     grad = logits.new_empty((T, E))
     with _on(dev):
         _lib.check(_lib.load().mxgg_route_topk_backward(
             logits.data_ptr(), _IN_DTYPES[logits.dtype], ld, T, E, k, int(routing.renormalise),
-            routing.experts.data_ptr(), routing.weights.data_ptr(), p + 4 * at[2], routing.counts.data_ptr(),
-            p + 4 * at[4] + 8, _addr(grad_weights), _addr(scalars[0]), coef[0], _addr(scalars[1]), coef[1],
+            p, p + 4 * at[1], p + 4 * at[2], p + 4 * at[3], p + 4 * at[4] + 8, _addr(grad_weights), _addr(scalars[0]), coef[0], _addr(scalars[1]), coef[1],
             grad.data_ptr(), _raw_stream(dev)), "mxgg_route_topk_backward")
     return grad
 
