@@ -203,7 +203,7 @@ WgradPlan wgrad_plan(int64_t M, int64_t C, int64_t R, int64_t L, int64_t S) {
   const int64_t tiles = wgrad_tiles(C);
   const int64_t stages = M > 0 && S > 0 ? ((M + kWgradBT - 1) / kWgradBT + std::min(S, M) - 1) * tiles : 0;
   w.ctas = std::min<int64_t>(stages, kWgradMaxCtas);
-  w.bytes = align256(stages > 0 ? (tiles * L + w.ctas) * kWgradBC * lora_rp((int)R) * 4 : 0);
+  w.bytes = align256(stages > 0 ? (tiles * wgrad_slots((int)L, (int)S) + w.ctas) * kWgradBC * lora_rp((int)R) * 4 : 0);
   return w;
 }
 
@@ -374,7 +374,8 @@ int mxgg_lora_mm(const void* x, int64_t x_ld, const void* a, const void* b, cons
 
 int64_t mxgg_lora_mm_backward_workspace_size(int64_t M, int64_t K, int64_t N, int64_t R, int64_t L,
                                              int64_t n_segments) {
-  if (M < 0 || M >= kExtent || K < 1 || N < 1 || R < 1 || R > kMaxLoraRank || R % 8 != 0 || L < 1 || n_segments < 0)
+  if (M < 0 || M >= kExtent || K < 1 || N < 1 || R < 1 || R > kMaxLoraRank || R % 8 != 0 || L < 1 || n_segments < 0 ||
+      K >= kExtent || N >= kExtent || L >= kExtent || n_segments > kMaxLoraSegments)
     return -1;
   return align256(v_bytes(M, R)) + wgrad_plan(M, K, R, L, n_segments).bytes +
          wgrad_plan(M, N, R, L, n_segments).bytes;

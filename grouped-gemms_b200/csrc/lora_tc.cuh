@@ -650,10 +650,14 @@ struct WgradJob {
   int ctas;                  // CTAs that share the axis (the first ones of the grid)
   int transposed;            // output (L, C, R) instead of (L, R, C)
   void* out;
-  // partial of (tile i, adapter l, CTA b): slot i * L + l + b, [128][Rp] floats; the slots of what occurs are
-  // distinct, as a step along the axis raises i * L + l or b
+  // partial of (tile i, adapter l, CTA b): slot i * slots + wgrad_slot(l) + b, [128][Rp] floats; the slots of what
+  // occurs are distinct, as a step along the axis raises i * slots + wgrad_slot(l) or b
   float* part;
 };
+// Slots of a tile: an adapter's own number, or, when there are more adapters than segments, the number of segments
+// with rows of lower ones.  A table of many adapters, of which a batch carries a few, takes no more than the few.
+__host__ __device__ constexpr int wgrad_slots(int L, int S) { return L < S ? L : S; }
+
 struct WgradParams {
   LoraSegs g;
   int R, Rp, stages;
@@ -668,7 +672,7 @@ constexpr int kWgradZBytes = kWgradBC * kWgradBT * 2;
 constexpr int kWgradMaxCtas = 2 * 148;   // two to an SM
 constexpr int kWgradThreads = 192;   // TMA, MMA, four epilogue warps
 
-__host__ __device__ constexpr int wgrad_table_bytes(int S) { return (5 * S + 2) * 4; }
+__host__ __device__ constexpr int wgrad_table_bytes(int S) { return (6 * S + 2) * 4; }
 __device__ __forceinline__ long long wgrad_cut(long long total, int b, int ctas) { return total * b / ctas; }
 
 __global__ void __launch_bounds__(kWgradThreads)
@@ -676,12 +680,14 @@ lora_wgrad_kernel(const __grid_constant__ CUtensorMap map_v0, const __grid_const
                   const __grid_constant__ CUtensorMap map_v1, const __grid_constant__ CUtensorMap map_z1,
                   const __grid_constant__ WgradParams p) {
   extern __shared__ uint8_t smem_raw[];
-  // tables of the segments: start and stages before (in order), adapter; by adapter: segment and stages before
+  // tables of the segments: start and stages before (in order), adapter; by adapter: segment, stages before, slot
   int* sh_start = reinterpret_cast<int*>(smem_raw);
   int* sh_tiles = sh_start + p.g.S + 1;
   int* sh_ad = sh_tiles + p.g.S + 1;
   int* sh_seg = sh_ad + p.g.S;
   int* sh_pre = sh_seg + p.g.S;
+  int* sh_slot = sh_pre + p.g.S;
+  const int slots = wgrad_slots(p.g.L, p.g.S);
   __shared__ int sh_n;
   __shared__ alignas(8) uint64_t sh_full[kWgradMaxStages], sh_empty[kWgradMaxStages];
   __shared__ alignas(8) uint64_t sh_acc_full[2], sh_acc_empty[2], sh_done;
@@ -724,16 +730,18 @@ lora_wgrad_kernel(const __grid_constant__ CUtensorMap map_v0, const __grid_const
   for (int s = tid; s < p.g.S; s += kWgradThreads) {
     const int l = sh_ad[s], n = sh_tiles[s + 1] - sh_tiles[s];
     if (l < 0 || n == 0) continue;
-    int rank = 0, pre = 0;
+    int rank = 0, pre = 0, lower = 0;
     for (int o = 0; o < p.g.S; ++o) {
       const int lo = sh_ad[o], no = sh_tiles[o + 1] - sh_tiles[o];
       if (lo >= 0 && no > 0 && (lo < l || (lo == l && o < s))) {
         ++rank;
         pre += no;
+        lower += lo < l;
       }
     }
     sh_seg[rank] = s;
     sh_pre[rank] = pre;
+    sh_slot[rank] = slots == p.g.L ? l : lower;
     atomicAdd(&sh_n, 1);
   }
   __syncthreads();
@@ -752,7 +760,7 @@ lora_wgrad_kernel(const __grid_constant__ CUtensorMap map_v0, const __grid_const
 
   // A run of stages in one segment and tile; every role walks the same runs.
   struct Run {
-    int tile, adapter, row, end, n;
+    int tile, adapter, slot, row, end, n;
     bool flush;                    // the accumulator ends with it
   };
   auto run = [&](long long t, long long t1) {
@@ -767,6 +775,7 @@ lora_wgrad_kernel(const __grid_constant__ CUtensorMap map_v0, const __grid_const
     }
     const int s = sh_seg[lo], after = lo + 1 < nseg ? sh_pre[lo + 1] : W;
     w.adapter = sh_ad[s];
+    w.slot = sh_slot[lo];
     w.row = sh_start[s] + (q - sh_pre[lo]) * kWgradBT;
     w.end = sh_start[s + 1];
     const long long left = t1 - t;
@@ -908,7 +917,7 @@ lora_wgrad_kernel(const __grid_constant__ CUtensorMap map_v0, const __grid_const
         const int c = q * 32 + lane;
         const bool in = w.tile * kWgradBC + c < p.job[jb].C;
         float* dst = p.job[jb].part +
-                     ((long long)w.tile * p.g.L + w.adapter + blockIdx.x) * (kWgradBC * p.Rp) + c * p.Rp;
+                     ((long long)w.tile * slots + w.slot + blockIdx.x) * (kWgradBC * p.Rp) + c * p.Rp;
         const uint32_t lane_addr = tmem + ((uint32_t)(q * 32) << 16) + buf * acc_cols;
         for (int r = 0; r < p.Rp; r += 16) {
           uint32_t a[16], b[16];
@@ -961,28 +970,31 @@ __global__ void __launch_bounds__(256) lora_wgrad_sum_kernel(const __grid_consta
   const int ld = p.Rp + 1;
   int* sh_start = reinterpret_cast<int*>(sh + ncols * ld);
   int* sh_tiles = sh_start + p.g.S + 1;
-  __shared__ int sh_before, sh_mine, sh_all;
+  __shared__ int sh_before, sh_mine, sh_all, sh_lower;
   __shared__ bool sh_has[kWgradMaxCtas];
   const int tid = threadIdx.x, lane = tid & 31;
   const int blocks0 = (p.job[0].C + ncols - 1) / ncols;
   const int which = (int)blockIdx.x >= blocks0;
   const WgradJob& job = p.job[which];
   const int c0 = ((int)blockIdx.x - (which ? blocks0 : 0)) * ncols, l = blockIdx.y;
-  if (tid == 0) sh_before = sh_mine = sh_all = 0;
+  if (tid == 0) sh_before = sh_mine = sh_all = sh_lower = 0;
   if (tid < 32) lora_build_table(p.g, kWgradBT, sh_start, sh_tiles);
   __syncthreads();
-  // stages of a column tile: of lower adapters, of this one, of all
-  int before = 0, mine = 0, all = 0;
+  // stages of a column tile: of lower adapters, of this one, of all; segments with rows of lower adapters
+  int before = 0, mine = 0, all = 0, lower = 0;
   for (int s = tid; s < p.g.S; s += 256) {
     const int a = lora_adapter(p.g, s), n = a < 0 ? 0 : sh_tiles[s + 1] - sh_tiles[s];
     all += n;
     before += a < l ? n : 0;
     mine += a == l ? n : 0;
+    lower += a < l && n > 0;
   }
   before = __reduce_add_sync(0xFFFFFFFFu, before);
   mine = __reduce_add_sync(0xFFFFFFFFu, mine);
   all = __reduce_add_sync(0xFFFFFFFFu, all);
+  lower = __reduce_add_sync(0xFFFFFFFFu, lower);
   if (lane == 0) {
+    atomicAdd(&sh_lower, lower);
     atomicAdd(&sh_before, before);
     atomicAdd(&sh_mine, mine);
     atomicAdd(&sh_all, all);
@@ -1003,7 +1015,9 @@ __global__ void __launch_bounds__(256) lora_wgrad_sum_kernel(const __grid_consta
   __syncthreads();
   ptx::griddep_wait();
   const int cols = min(ncols, job.C - c0), quads = p.Rp / 4;
-  const float* part = job.part + ((long long)tile * p.g.L + l) * (kWgradBC * p.Rp) + (long long)(c0 % kWgradBC) * p.Rp;
+  const int slots = wgrad_slots(p.g.L, p.g.S);
+  const float* part = job.part + ((long long)tile * slots + (slots == p.g.L ? l : sh_lower)) * (kWgradBC * p.Rp) +
+                      (long long)(c0 % kWgradBC) * p.Rp;
   for (int e = tid; e < cols * quads; e += 256) {
     const int c = e / quads, r = (e % quads) * 4;
     float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
