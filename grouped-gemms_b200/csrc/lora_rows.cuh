@@ -248,7 +248,7 @@ __global__ void __launch_bounds__(KC <= 4 ? kRowsMaxThreads : 256) lora_rows_ker
       for (int kc = 0; kc < KC; ++kc) {
         const uint2 u = kc * 16 + 4 * t < p.R ? w[j][kc] : make_uint2(0, 0);
         ptx::mma_m16n8k16_bf16(d[j], hi[kc][0], hi[kc][1], hi[kc][2], hi[kc][3], u.x, u.y);
-        ptx::mma_m16n8k16_bf16(d[j], lo[kc][0], lo[kc][1], lo[kc][2], lo[kc][3], u.x, u.y);
+        ptx::mma_m16n8k16_bf16(d[j], lo[kc][0], lo[kc][1], lo[kc][2], lo[kc][3], finite_pair(u.x), finite_pair(u.y));
       }
     }
     const int c = gi * 32 + t * 8;

@@ -88,6 +88,12 @@ __device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t&
   hi = pack_bf16(a, b);
   lo = pack_bf16(low_half(a, __uint_as_float(hi << 16)), low_half(b, __uint_as_float(hi & 0xFFFF0000u)));
 }
+// Beside an infinite weight the high half alone gives the product (it has v's sign, and is 0 where v is); the low
+// half's own sign, or its 0, would make a NaN of it.  So the low half is multiplied by a packed pair of weights with 0
+// for infinities and NaNs.
+__device__ __forceinline__ uint32_t finite_pair(uint32_t w) {
+  return w & ~(((((w & 0x7F807F80u) + 0x00800080u) >> 15) & 0x00010001u) * 0xFFFFu);
+}
 // Eight values as v's two halves, 16 bytes each.
 __device__ __forceinline__ void split_halves(const float (&f)[8], uint4& hi, uint4& lo) {
   uint32_t h[4], l[4];
@@ -333,7 +339,10 @@ __global__ void __launch_bounds__(128) lora_shrink_kernel(const __grid_constant_
 // of four epilogue warps take tiles in turn: they add the base in place in
 // shared memory and store the tile by TMA (32 full rows of a warp) or row by
 // row (rows that end inside).  Two groups, as one spends most of a tile waiting
-// (accumulator, shared memory, its store's read of the stage).
+// (accumulator, shared memory, its store's read of the stage).  A product that
+// comes out NaN is taken again from shared memory, infinite weights times v's high
+// half alone (finite_pair): looking through the weights before the products took 1
+// to 30 % of the kernel (ranks 16 to 128), looking for NaNs afterwards none.
 // Bound: HBM, the base's read and the output's write.  16384 x 8192, rank 16:
 // 90 us, 6.0 TB/s.  One epilogue group with CTAs for 2.3 rounds took 185 us.
 struct ExpandParams {
@@ -365,6 +374,38 @@ __device__ __forceinline__ uint32_t lora_v_off(int Rp, int h, int j, uint32_t ti
   return (uint32_t)(h * ((Rp + 63) / 64) + j / 4) * tile + (uint32_t)(j % 4) * 32;
 }
 
+__device__ __forceinline__ float lds_bf16(uint32_t a) {
+  unsigned short u;
+  asm volatile("ld.shared.u16 %0, [%1];" : "=h"(u) : "r"(a));
+  return __uint_as_float((uint32_t)u << 16);
+}
+// Byte `at` of a tile in the swizzle pattern of `row` (32, 64 or 128) bytes.
+__device__ __forceinline__ uint32_t swizzled(uint32_t at, uint32_t row) {
+  return at ^ (((at >> 7) & (row / 16 - 1)) << 4);
+}
+// v W^T of row r and column c of a tile, infinite weights times v's high half alone.  It ends at the first NaN:
+// whole adapters of them would take milliseconds.
+__device__ __noinline__ float lora_product(uint32_t vbuf, uint32_t ws, int Rp, int r_contig, int w_row, int r, int c) {
+  float sum = 0.0f;
+  for (int k = 0; k < Rp && !isnan(sum); ++k) {
+    const uint32_t at = lora_v_off(Rp, 0, k / 16, kLoraBM * 128) + k % 16 * 2, high = swizzled(at + r * 128, 128);
+    const uint32_t al = lora_v_off(Rp, 1, k / 16, kLoraBM * 128) + k % 16 * 2, low = swizzled(al + r * 128, 128);
+    const float w = lds_bf16(ws + (r_contig ? (k / 64) * (kExpandBN * 128) + swizzled(c * w_row + k % 64 * 2, w_row)
+                                            : swizzled(k * 128 + c * 2, 128)));
+    sum = fmaf(lds_bf16(vbuf + high), w, sum);
+    if (isfinite(w)) sum = fmaf(lds_bf16(vbuf + low), w, sum);
+  }
+  return sum;
+}
+
+// NaN if one of the values is.
+__device__ __forceinline__ float any_nan(const uint32_t (&a)[32]) {
+  float m = __uint_as_float(a[0]);
+#pragma unroll
+  for (int i = 1; i < 32; ++i) asm("max.NaN.f32 %0, %0, %1;" : "+f"(m) : "f"(__uint_as_float(a[i])));
+  return m;
+}
+
 template <typename O>
 __device__ __forceinline__ void lora_add8(float (&f)[8], const uint4& q) {
   if constexpr (sizeof(O) == 2) {
@@ -374,8 +415,9 @@ __device__ __forceinline__ void lora_add8(float (&f)[8], const uint4& q) {
   }
 }
 
+// Two to an SM: left alone the compiler takes 64 registers and spills in the loop (117 us instead of 101, rank 32).
 template <typename O>
-__global__ void __launch_bounds__(kExpandThreads)
+__global__ void __launch_bounds__(kExpandThreads, 2)
 lora_expand_kernel(const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_w,
                    const __grid_constant__ CUtensorMap map_base, const __grid_constant__ CUtensorMap map_base32,
                    const __grid_constant__ CUtensorMap map_out, const ExpandParams p) {
@@ -552,6 +594,15 @@ lora_expand_kernel(const __grid_constant__ CUtensorMap map_v, const __grid_const
         uint32_t a[32];
         ptx::tmem_ld_32x32b_x32(lane_addr + buf * kExpandBN + half * 32, a);
         ptx::tmem_wait_ld();
+        if (__any_sync(0xFFFFFFFFu, isnan(any_nan(a)) && mine)) {
+          ptx::mbar_wait(ptx::smem_u32(&sh_v), 0, abort, p.wait_ns);   // long done: these threads see v by it
+          const uint32_t ws = ring + st * stage_bytes + p.base_bytes;
+#pragma unroll
+          for (int u = 0; u < 32; ++u)
+            if (isnan(__uint_as_float(a[u])) && mine)
+              a[u] = __float_as_uint(lora_product(vbuf, ws, p.Rp, p.r_contig, p.w_row, r, half * 32 + u));
+          __syncwarp();
+        }
 #pragma unroll
         for (int u = 0; u < 32; u += kPer16) {
           const int col = half * 32 + u;
@@ -639,7 +690,10 @@ lora_expand_kernel(const __grid_constant__ CUtensorMap map_v, const __grid_const
 // then writes an fp32 partial; a second launch adds a block's partials in CTA
 // order.  Loads run ahead across those ends.  Rows of a stage past its segment's
 // end belong to others: they are zeroed in shared memory, as 0 * NaN would not
-// be 0.
+// be 0.  Where v's halves have accumulators of their own (Rp <= 32) the low one's
+// sum counts only where it is finite: beside an infinite z the high one's is the
+// result (finite_pair).  Above, an infinite z gives NaN for an infinity; sums of
+// their own took 6 to 14 % of the kernel there (ranks 64 and 128).
 // Bound: HBM, z once (two CTAs to an SM keep 128 KB of it on the way).  16384
 // rows, 5120 + 8192 columns, rank 16 (436 MB): 87 us, 5.0 TB/s, and 6 us for the
 // sums; one CTA to an SM took half as long again, its products' issue and waits
@@ -927,7 +981,10 @@ lora_wgrad_kernel(const __grid_constant__ CUtensorMap map_v0, const __grid_const
           if (in) {
             if (joined)
 #pragma unroll
-              for (int i = 0; i < 16; ++i) a[i] = __float_as_uint(__uint_as_float(a[i]) + __uint_as_float(b[i]));
+              for (int i = 0; i < 16; ++i) {
+                const float l = __uint_as_float(b[i]);
+                a[i] = __float_as_uint(__uint_as_float(a[i]) + (isfinite(l) ? l : 0.0f));
+              }
 #pragma unroll
             for (int i = 0; i < 16; i += 4)
               *reinterpret_cast<uint4*>(dst + r + i) = make_uint4(a[i], a[i + 1], a[i + 2], a[i + 3]);

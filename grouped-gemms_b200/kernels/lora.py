@@ -85,6 +85,8 @@ def lora_grouped_mm_backward(
     ``grad_a`` ``(L, R, K)`` and ``grad_b`` ``(L, N, R)`` of ``grad_w_dtype`` (bf16, fp16 or fp32) sum over
     every row that carries the adapter (zeros where none does), in an order that does not depend on timing.
     ``need`` says which of the three are wanted; the others come back empty.
+    Infinite elements give the formula's infinities, except that at ranks above 32 those of ``x`` in ``grad_a`` and of
+    ``grad_out`` in ``grad_b`` may give NaN instead.
     """
     if not _mxfp8_available:
         raise NotImplementedError(_UNAVAILABLE_MSG)

@@ -514,6 +514,8 @@ int mxgg_lora_mm(const void* x, int64_t x_ld, const void* a, const void* b, cons
  *   grad_a (L, R, K), grad_b (L, N, R) of grad_w_dtype: sums over every row
  *            that carries the adapter, in a fixed order; zeros for an adapter
  *            that no row carries
+ * Infinite elements give the formula's infinities, except that at ranks above
+ * 32 those of x in grad_a and of grad_out in grad_b may give NaN instead.
  * Each may be null (not computed); x is needed for grad_a, v for grad_b.
  * Outputs overlap no other operand.
  * Segments are needed (not the row form).  workspace: at least
