@@ -33,8 +33,9 @@ def lora_grouped_mm(
     Args:
         x: ``(M, K)`` bf16 (the unquantised input of the projection).
         lora_a: ``(L, R, K)`` bf16; lora_b: ``(L, N, R)`` bf16.  K, N and R multiples of 8, R <= 128.
-        group_end_offsets: ``(S,)`` cumulative row ends of the segments (at most 1024), or ``None``: every
-            row is a segment of its own (a decode step's rows).
+        group_end_offsets: ``(S,)`` int32 / int64 cumulative row ends of the segments (at most 1024; cut at M),
+            or ``None``: every row is a segment of its own.  That form is for a decode step: a row looks for its
+            adapter's others among 1024, and thousands of rows take ten times as long as in segments.
         adapter: ``(S,)`` int32 / int64 adapter of each segment; a value outside ``[0, L)`` (say -1) means
             none.  ``None``: segment s carries adapter s.
         scaling: ``(L,)`` fp32 factor of each adapter, ``None``: 1.

@@ -518,6 +518,8 @@ def _lora_args(what: str, x: Tensor, a: Tensor, b: Tensor, offs: Optional[Tensor
         if offs.dim() != 1:
             raise ValueError(f"{what}: group_end_offsets must have one dimension")
         S = offs.shape[0]
+        if offs.dtype == torch.int64:
+            offs = offs.clamp(0, M)          # an end that int32 does not hold must not wrap into the rows
         offs = _as(offs, torch.int32)
     if adapter is not None:
         if adapter.dtype == torch.int64:
