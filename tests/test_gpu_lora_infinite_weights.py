@@ -82,3 +82,65 @@ def test_nan_weights_stay_in_their_columns():
     assert bool(out[:200].isnan().all()) and bool(out[200:, 700].isnan().all())
     keep = [c for c in range(1032) if c != 700]
     assert torch.equal(out[200:, keep], clean[200:, keep])
+
+
+def signs(M, K, N, R, seed=9):
+    """Operands of both signs, and which of v's elements are far enough from 0 to have a sign beyond doubt."""
+    from test_gpu_lora import make, reference
+    x, a, b, s, base = make(M, K, N, R, 2, seed=seed)
+    rows = torch.zeros(M, dtype=torch.int64, device="cuda")
+    rows[M // 2:] = 1
+    v, verr, _, _ = reference(x, a, b, s, None, rows)
+    return x, a, b, s, base, rows, v, v.abs() > 2 * verr
+
+
+@pytest.mark.parametrize("M", [24, 300])
+@pytest.mark.parametrize("R", RANKS)
+def test_signs_of_infinities(M, R):
+    """An infinite weight in every column, of either sign and at every rank: the infinity has v's sign times the
+    weight's.  Two of them in a column: an infinity where their signs agree, NaN where they do not."""
+    import kernels
+    K, N = 64, 200
+    x, a, b, s, base, rows, v, sure = signs(M, K, N, R)
+    ends, ad = cuda_i32([M // 2, M]), cuda_i32([0, 1])
+    cols = torch.arange(N, device="cuda")
+    first, second = cols % R, (7 * cols + 3) % R
+    one, two = b.clone(), b.clone()
+    up = torch.where(cols % 3 == 0, -INF, INF)
+    for l in range(2):
+        one[l, cols, first] = up.bfloat16()
+        two[l, cols, first] = up.bfloat16()
+        two[l, cols, second] = INF
+    p, q = v[:, first] * up, v[:, second] * INF
+    known, both = sure[:, first], sure[:, first] & sure[:, second]
+    p2 = torch.where(first == second, q, p)
+    for w, want, ok in ((one, p, known), (two, p2 + q, both)):
+        for out in (kernels.lora_grouped_mm(x, a, w, ends, ad, s, base=base),
+                    kernels.lora_grouped_mm(x, a, w, None, rows.int(), s, base=base, out_dtype=base.dtype)):
+            got = out.double()
+            same = (got == want) | (got.isnan() & want.isnan())
+            assert bool(same[ok].all()), int((~same & ok).sum())
+
+
+@pytest.mark.parametrize("R", [8, 24, 32])
+def test_signs_of_infinities_in_a_weight_gradient(R):
+    """An infinite x in every seventh column: grad_a's infinity has dv's sign times its own."""
+    import kernels
+    M, K, N = 400, 200, 136
+    x, a, b, s, _, rows, _, _ = signs(M, K, N, R)
+    from test_gpu_lora import reference
+    ends, ad = cuda_i32([M // 2, M]), cuda_i32([0, 1])
+    go = torch.randn(M, N, generator=torch.Generator().manual_seed(5)).bfloat16().cuda()
+    dv, err, _, _ = reference(go, b.transpose(1, 2).contiguous(), a.transpose(1, 2).contiguous(), s, None, rows)
+    _, v = kernels.lora_grouped_mm(x, a, b, ends, ad, s, return_v=True)
+    x2 = x.clone()
+    for c in range(0, K, 7):
+        m = M // 2 + 3 * c // 7 % 200
+        x2[m, c] = INF if c % 2 else -INF
+    _, ga, _ = kernels.lora_grouped_mm_backward(go, x2, a, b, v, ends, ad, s, need=(False, True, False))
+    for c in range(0, K, 7):
+        m = M // 2 + 3 * c // 7 % 200
+        ok = dv[m].abs() > 2 * err[m]
+        assert torch.equal(ga[1, :, c].double()[ok], (dv[m] * (INF if c % 2 else -INF))[ok])
+    rest = [c for c in range(K) if c % 7]
+    assert bool(ga[:, :, rest].isfinite().all()) and bool(ga[0].isfinite().all())
