@@ -147,7 +147,8 @@ int expand_as(DeviceState* st, const LoraSegs& g, const void* v, const void* w, 
   p.wait_ns = wait_limit_ns();
   const long long tiles = ((long long)g.M + kLoraBM - 1) / kLoraBM + std::min(g.S, g.M) - 1;
   const int nt = (int)((C + kExpandBN - 1) / kExpandBN);
-  // Cut the columns until the CTAs (two to an SM) fill the GPU once, each keeping two tiles (v is loaded once per CTA).
+  // Cut the columns until two CTAs to an SM fill the GPU once, each keeping two tiles (v is loaded once per CTA).  Where
+  // one fits (fp32 results; 16-bit ones above rank 32, grad_x above 48) they come in two rounds.
   p.nsplit = (int)std::max<long long>(1, std::min<long long>((nt + 1) / 2, 2LL * st->num_sms / tiles));
   const int vb = p.v_pieces * kLoraBM * 128, stage = p.base_bytes + p.w_bytes;
   // two CTAs share an SM where that leaves each three stages

@@ -68,7 +68,7 @@ bool route_vec(const void* p, int64_t ld, int64_t E, int es) {
 }
 
 template <typename T, int G, int V>
-int launch_route(const RouteParams& p, int num_sms, cudaStream_t stream) {
+int launch_route(const RouteParams& p, int, cudaStream_t stream) {
   const RouteShape s = route_shape(p.T, p.E);
   route_topk_kernel<T, G, V><<<s.blocks, s.warps * 32, 0, stream>>>(p);
   MXGG_CUDA_TRY(cudaGetLastError());

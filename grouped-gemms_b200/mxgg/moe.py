@@ -386,21 +386,20 @@ class MoELayer:
             # the up projection's epilogue writes to_mx of its bf16 output
             h_s, h_q, _, _, _ = grouped_mm_mx(a_q, self.up_q, a_s, self.up_s, lay.offs, seg_e, torch.bfloat16, False)
             y = grouped_mm_segments(h_q, self.down_q, h_s, self.down_s, lay.offs, seg_e, torch.bfloat16)
-        else:
-            layout = dispatch_layout(experts, self.n_experts)
-            a_s, a_q = quantize_gather(x, layout.row_index)
-            # rows stream into the hosts' receive buffers while the up projection
-            # consumes them; the down projection sends its rows to their owners
-            ep = self.ep
-            plan = ep.plan(layout.counts, self.placement)
-            ep.dispatch(plan, a_q, a_s)
-            h_q = torch.empty((plan.rows_recv, self.d_ff), dtype=torch.float8_e4m3fn, device=x.device)
-            h_s = torch.empty((plan.rows_recv, self.d_ff // 32), dtype=torch.uint8, device=x.device)
-            ep.gemm_received(plan, self.d_model, self.up_q, self.up_s, torch.bfloat16, local_mx=(h_q, h_s))
-            ep.gemm_local(plan, h_q, h_s, self.down_q, self.down_s, torch.bfloat16)
-            y = ep.finish(plan, self.d_model, torch.bfloat16)
-            return combine_top2(y, layout, weights)
-        return combine_topk(y, lay.pair_pos, weights)
+            return combine_topk(y, lay.pair_pos, weights)
+        layout = dispatch_layout(experts, self.n_experts)
+        a_s, a_q = quantize_gather(x, layout.row_index)
+        # rows stream into the hosts' receive buffers while the up projection
+        # consumes them; the down projection sends its rows to their owners
+        ep = self.ep
+        plan = ep.plan(layout.counts, self.placement)
+        ep.dispatch(plan, a_q, a_s)
+        h_q = torch.empty((plan.rows_recv, self.d_ff), dtype=torch.float8_e4m3fn, device=x.device)
+        h_s = torch.empty((plan.rows_recv, self.d_ff // 32), dtype=torch.uint8, device=x.device)
+        ep.gemm_received(plan, self.d_model, self.up_q, self.up_s, torch.bfloat16, local_mx=(h_q, h_s))
+        ep.gemm_local(plan, h_q, h_s, self.down_q, self.down_s, torch.bfloat16)
+        y = ep.finish(plan, self.d_model, torch.bfloat16)
+        return combine_top2(y, layout, weights)
 
     def flops(self, tokens: int) -> float:
         """Useful FLOPs of one forward over `tokens` tokens (padding excluded)."""
