@@ -14,7 +14,7 @@
 // experts; for many the selection's integer instructions.  65521 tokens, 256
 // experts, top-8, bf16: forward 35 us (34 MB; the integer pipe is the busiest,
 // issue slots 64 %), the losses' sums 7 us, backward 22 us (67 MB, 3.1 TB/s).
-// 16384 tokens, 8 experts, top-2, fp32: 4.2, 3.5 and 3.7 us.
+// 16384 tokens, 8 experts, top-2, fp32: 4.3, 4.9 (its start overlapped) and 3.5 us.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -126,7 +126,9 @@ __device__ __forceinline__ float route_exp(float d) {
   // beside an infinite d, 0 as it is; a NaN stays one through r
   return d > -126.0f ? fmaf(r, e * kLn2, r) : r;
 }
-// exp(d - s), s_log2e = s log2(e), for sums and gradients: off by |d| 2^-24.
+// exp(d - s), s_log2e = s log2(e), for the gradient and, beyond 128 experts, the sums: off by (|d| + |s|) 2^-24 and
+// the 2 ulp of 2^x, tiny results flushed to 0.  The rounding of d = x - max alone is |d| 2^-24 of the result, in
+// whatever exponential: the gradient of 16384 x 8 is 9.9e-8 of its norm off float64, 9.5e-8 in plain fp32 operations.
 __device__ __forceinline__ float route_exp(float d, float s_log2e) {
   return route_ex2(fmaf(d, 1.44269504089f, -s_log2e));
 }

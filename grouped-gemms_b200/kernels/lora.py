@@ -47,6 +47,9 @@ def lora_grouped_mm(
 
     Rows without an adapter are ``base``'s (zeros without one); rows at or past the last end are left
     unwritten, like ``triton_mxfp8_grouped_mm``'s.
+
+    The intermediate ``v = scaling x lora_a^T`` is an fp32 sum kept in two bf16 halves, 16 bits of mantissa: an fp32
+    result carries an error of up to 2^-17 of ``sum |v lora_b|``, not fp32's own.
     """
     if not _mxfp8_available:
         raise NotImplementedError(_UNAVAILABLE_MSG)

@@ -421,7 +421,8 @@ int mxgg_combine_topk(const void* y, int64_t y_rows, const int64_t* pos, const f
  *            mean of (log sum exp)^2.  Both 0 when no token counts.
  *   n_counted  1 int32: n
  * A NaN or +inf logit of a counted token makes its weights and both losses
- * NaN; its choices are still valid experts (NaN ranks above +inf).  Sums run in a fixed order: results do not depend on timing.
+ * NaN; its choices are still valid experts (NaN ranks above +inf).  Sums run in
+ * a fixed order: results do not depend on timing.
  * experts <= 1024, k <= min(experts, 16).  workspace: at least
  * mxgg_route_workspace_size bytes, 16-byte aligned.  No counterpart in the
  * reference.
@@ -492,14 +493,15 @@ int mxgg_dispatch_backward(const void* grad_rows, int64_t rows, const int64_t* p
  *            same row stride), so that the product is added in place
  *   out (M, N) of out_dtype (MXGG_DTYPE_*): rows without an adapter take
  *            base's; rows at or past the last end are not written
- *   v        mxgg_lora_v_bytes(M, R) bytes: the scaled intermediate in fp32
- *            precision of 16 bits (two bf16 halves), which the backward pass
- *            takes; 0 for rows without an adapter.  May be null without
- *            segment_end_offsets (single rows)
+ *   v        mxgg_lora_v_bytes(M, R) bytes: the scaled intermediate, an fp32
+ *            sum kept in 16 bits of mantissa (two bf16 halves), which the
+ *            backward pass takes; 0 for rows without an adapter.  So fp32
+ *            results carry an error of up to 2^-17 of sum |v b|, not fp32's
+ *            own.  May be null without segment_end_offsets (single rows)
  * segment_end_offsets null (n_segments = M): every row is a segment of its
  * own, the form of a decode step.  Sums are fp32.  K, N and R multiples of 8,
- * R <= 128, at most 1024 segments and 65535 adapters; rows 16-byte aligned.  No counterpart in
- * the reference.
+ * R <= 128, at most 1024 segments and 65535 adapters; rows 16-byte aligned.
+ * No counterpart in the reference.
  */
 int64_t mxgg_lora_v_bytes(int64_t M, int64_t R);
 int mxgg_lora_mm(const void* x, int64_t x_ld, const void* a, const void* b, const int32_t* segment_end_offsets,
